@@ -17,7 +17,6 @@ tokens, vocabularies of 248320 and 65536 are this repository's own; the other he
 """
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -31,7 +30,6 @@ DEV, BF, F32, F64 = "cuda", torch.bfloat16, torch.float32, torch.float64
 PAGE, THETA = 16, 1e7
 
 
-@functools.cache                                # a user's program imports once
 def _ops():
     root = str(Path(__file__).resolve().parent.parent / "qwen3_5-triton-inference-engine_b200")
     if root not in sys.path:
