@@ -106,10 +106,10 @@ int b200_paged_kv_append_rope(const b200_rope_append_args* args, b200_stream_t s
  * tokens of the sequence, its own key and value (already in the cache) being the last.  out [T, H_q * D] = softmax(q k / sqrt(D)) v,
  * times sigmoid(gate) where gate [T, H_q * D] is not NULL.  q is rotated already (b200_paged_kv_append_rope).  One token per sequence is
  * a decode step, a few are the check of a speculated continuation, hundreds a portion of a prompt; a sequence may have none.
- * D 128 or 256, 1 to 64 Q heads per KV head; strides multiples of 8 elements.  Rows outside [cu_seqlens[0], cu_seqlens[batch]) of out are
- * left as they are.  A table entry outside [0, num_pages) reads as zeros.  What the last page holds behind the sequence's end has no
- * influence, not even infinities and NaN.  For a call alone while it runs: workspace, b200_paged_gqa_attention_chunk_workspace_bytes(D)
- * bytes of any content, 16-byte aligned.
+ * D 128 or 256, 1 to 64 Q heads per KV head; strides multiples of 8 elements.  cu_seqlens ascends; below zero it names a sequence whose first
+ * tokens are in the cache but not among the rows.  Rows outside [cu_seqlens[0], cu_seqlens[batch]) of out are left as they are.  A table
+ * entry outside [0, num_pages) reads as zeros.  What the last page holds behind the sequence's end has no influence, not even infinities and
+ * NaN.  For a call alone while it runs: workspace, b200_paged_gqa_attention_chunk_workspace_bytes(D) bytes of any content, 16-byte aligned.
  * (The reference prefills from position 0 only: gqa_attention_varlen_causal.py:214.) */
 int64_t b200_paged_gqa_attention_chunk_workspace_bytes(int32_t head_dim);
 typedef struct { /* 8-byte fields only */

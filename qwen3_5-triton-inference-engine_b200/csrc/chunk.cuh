@@ -47,8 +47,10 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int b) {
   const int from = p.cu_seqlens[b], to = min(p.cu_seqlens[b + 1], p.tokens);
   q.start = max(from, 0);
   q.n = max(to - q.start, 0);
-  const int64_t held = p.pos[b], room = static_cast<int64_t>(p.max_pages) * PAGE;
-  q.s = static_cast<int>(min(max(held, static_cast<int64_t>(0)), min(room, static_cast<int64_t>(1) << 30) - 1));
+  // (a sequence that begins in front of the packed rows: its tokens there are as good as held)
+  const int64_t most = min(static_cast<int64_t>(p.max_pages) * PAGE, static_cast<int64_t>(1) << 30) - 1;
+  const int64_t held = min(max(p.pos[b], static_cast<int64_t>(0)), most) + (q.start - static_cast<int64_t>(from));
+  q.s = static_cast<int>(min(held, most));
   return q;
 }
 // Length of the first j blocks of one head, all of them whole; j below the number of blocks.
