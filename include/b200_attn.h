@@ -472,9 +472,9 @@ int b200_argmax_rows(const float* logits, int64_t row_stride, int64_t* ids, void
  *   shortest of these prefixes of the order: the first top_k; those with w >= min_p; the fewest whose weights reach top_p of the sum over
  *   what the other two kept.  The first token is always kept.  top_k <= 0 or >= n, min_p <= 0 and top_p >= 1 keep everything.  The id is
  *   the first kept token, by index, at which the running sum of kept weights exceeds uniform times their sum.
- * n up to 524288.  temperature <= 0 or NaN: the largest, ties to the lowest index (as b200_argmax_rows); below 1e-6 it counts as 1e-6.  Several
- * infinities share everything; a row of nothing but -inf and NaN gives 0.  Sums are exact to 2^-31 of a weight, so equal calls give equal
- * ids.  temperature, top_k, top_p, min_p: device arrays [rows], or NULL for the `_all` value.
+ * n up to 524288.  temperature <= 0 or NaN: the largest, ties to the lowest index (as b200_argmax_rows); below 1e-6 it counts as 1e-6, infinity
+ * as the largest float.  Several infinities share everything; a row of nothing but -inf and NaN gives 0.  Sums are exact to 2^-31 of a weight, so
+ * equal calls give equal ids.  temperature, top_k, top_p, min_p: device arrays [rows], or NULL for the `_all` value.
  * (The reference only has the arg-max: vocab_argmax.py:141-200.) */
 typedef struct { /* 8-byte fields only */
   const void* logits;

@@ -221,7 +221,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
   best = -INFINITY;
   for (int i = 0; i < csize; ++i) best = fmaxf(best, __uint_as_float(sm.cta_max[i]));
 
-  const float temp = fminf(fmaxf(temperature, 1e-6f), 1e36f);
+  const float temp = fminf(fmaxf(temperature, 1e-6f), 3.402823466e38f);  // (infinity as the largest float: c and the borders below stay finite)
   const bool greedy = !(temperature > 0.f) || best == -INFINITY;
   RowWeights weight;
   weight.table = sm.table;
