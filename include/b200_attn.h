@@ -84,8 +84,9 @@ int b200_paged_kv_append(void* k_cache, void* v_cache, int64_t kc_stride_p, int6
  * position_ids[t] (int32 or int64), or with axes > 1 position_ids[a * ids_stride_a + t] with a = freq_axis[i] (int32, [rotary_dim/2])
  * for frequency i: time, height and width of images and video in any order of the frequencies.  The angle is formed in 64 bits.
  * q / q_out [T, H_q, D], k / v [T, H_kv, D], caches [num_pages, H_kv, 16, D] bf16 with any strides that are multiples of 8; D and
- * rotary_dim multiples of 16, D <= 512.  q_out may be q.  Rows in front of cu_seqlens[0] and from cu_seqlens[batch] on are left as they
- * are; k and v of a token whose table entry lies outside [0, num_pages), or whose index is outside the table, are not written.
+ * rotary_dim multiples of 16, D <= 512.  q_out may be q.  cu_seqlens ascends; below zero it names a sequence whose first tokens are in the
+ * cache but not among the rows.  Rows in front of cu_seqlens[0] and from cu_seqlens[batch] on are left as they are; k and v of a token whose
+ * table entry lies outside [0, num_pages), or whose index is outside the table, are not written.
  * (The reference rotates and appends one token at a time: partial_rope.py:145, gqa_attention_decode_paged.py:254-305.) */
 typedef struct { /* 8-byte fields only */
   const void *q, *k, *v;

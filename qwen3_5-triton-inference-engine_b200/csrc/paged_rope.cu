@@ -80,8 +80,9 @@ rope_append_kernel(const __grid_constant__ RopeAppendParams p) {
     const int t = t0 + i, b = sequence_of(p.cu_seqlens, p.batch, t, lane);
     if (lane == 0) {
       int64_t page = -2;
-      if (b >= 0) {
-        const int64_t at = p.pos[b] + t - p.cu_seqlens[b];
+      const int begins = b >= 0 ? p.cu_seqlens[b] : 0;
+      if (b >= 0 && begins <= t) {  // (else cu_seqlens does not ascend, and the place would be a held token's)
+        const int64_t at = p.pos[b] + t - begins;
         page = -1;
         if (at >= 0 && at / PAGE < p.max_pages) page = p.block_table[b * p.bt_b + at / PAGE];
         if (page < 0 || page >= p.num_pages) page = -1;

@@ -40,3 +40,16 @@ def test_first_sequence_begins_in_front_of_the_rows(ops, new, held, gone, hkv, g
     ops.paged_kv_append_rope(u["q"], k[gone:], v[gone:], kc, vc, u["table"], u["cu"], u["pos"],
                              torch.arange(out.shape[0], device=DEV), freq, 64)
     assert torch.equal(kc, t["k_cache"]) and torch.equal(vc, t["v_cache"])
+
+
+@pytest.mark.parametrize("cu", [[150, 100, 200], [40, 0, 200, 90], [199, 120, 60, 1, 200]])
+def test_lengths_that_do_not_ascend_touch_no_held_token(ops, cu):
+    """Not a call with a meaning, but what sequences hold already stays as it is."""
+    held = [300] * (len(cu) - 1)
+    t = make_batch([200] * len(held), held, 2, 4, 256, seed=len(cu), device=DEV, junk=0.0, cached=False)
+    before = t["k_cache"].clone(), t["v_cache"].clone()
+    ops.paged_kv_append_rope(t["q"][:200], t["k"][:200], t["v"][:200], t["k_cache"], t["v_cache"], t["table"],
+                             torch.tensor(cu, dtype=torch.int32, device=DEV), t["pos"], torch.arange(200, device=DEV), torch.ones(32, device=DEV), 64)
+    for b, h in enumerate(held):
+        for cache, old in zip((t["k_cache"], t["v_cache"]), before):
+            assert torch.equal(cached_rows(cache, t["table"], b, h), cached_rows(old, t["table"], b, h))
