@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from chunk_helpers import BF, attention64, attention_tolerance, cached_rows, make_batch
+from chunk_helpers import BF, attention64, attention_tolerance, cached_rows, make_batch, sequences
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -53,3 +53,22 @@ def test_lengths_that_do_not_ascend_touch_no_held_token(ops, cu):
     for b, h in enumerate(held):
         for cache, old in zip((t["k_cache"], t["v_cache"]), before):
             assert torch.equal(cached_rows(cache, t["table"], b, h), cached_rows(old, t["table"], b, h))
+
+
+@pytest.mark.parametrize("new,held,rows,hkv,group,dim", [([5, 3], [20, 0], 6, 2, 4, 256), ([2, 3, 9], [300, 41, 7], 4, 2, 2, 128),
+                                                         ([90, 40], [333, 64], 70, 2, 4, 256), ([100, 500, 400], [20, 1500, 3], 190, 4, 3, 128)])
+def test_lengths_that_name_more_rows_than_there_are(ops, new, held, rows, hkv, group, dim):
+    """The rows that are there come out as in the whole batch, and they alone are appended."""
+    t = make_batch(new, held, hkv, group, dim, seed=rows, device=DEV, junk=0.0)
+    want, spread = attention64(t, t["gate"])
+    out = ops.paged_gqa_attention_chunk(t["q"][:rows], t["k_cache"], t["v_cache"], t["table"], t["cu"], t["pos"], gate=t["gate"][:rows])
+    worst = ((out.double() - want[:rows]).abs() / attention_tolerance(want, spread)[:rows]).max().item()
+    assert out.shape[0] == rows and worst <= 1, worst
+    vc = t["v_cache"].clone()
+    ops.paged_kv_append_rope(t["q"][:rows], t["k"][:rows], t["v"][:rows], t["k_cache"].clone(), vc, t["table"], t["cu"], t["pos"],
+                             torch.arange(rows, device=DEV), torch.ones(32, device=DEV), 64)
+    for b, first, n, h in sequences(t):
+        there = max(0, min(n, rows - first))
+        got, old = cached_rows(vc, t["table"], b, h + n), cached_rows(t["v_cache"], t["table"], b, h + n)
+        assert torch.equal(got[h: h + there], t["v"][first: first + there].double())
+        assert torch.equal(got[:h], old[:h]) and torch.equal(got[h + there:], old[h + there:])
