@@ -184,10 +184,11 @@ __device__ __forceinline__ void cp_async16(void* dst_smem, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst_smem)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }  // all but the newest N groups
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// The same, all but the newest N of them.
+// All but the newest N groups of them.
+template <int N>
+__device__ __forceinline__ void cp_async_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// bulk_wait_read, all but the newest N of the stores.
 template <int N>
 __device__ __forceinline__ void bulk_wait_read_but() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 // Barrier among `count` threads (a multiple of 32) that all name the same id (1..15; 0 is __syncthreads).
@@ -307,13 +308,9 @@ __device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float a, float b
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
-// The same location's address in the CTA of rank `rank`, and access to it there, for kernels whose CTAs write to one another's shared memory
-// in bulk (tests/test_peer_rules_cpu.py holds the rules for them).
-__device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) {
-  uint32_t out;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_u32(p)), "r"(rank));
-  return out;
-}
+// cluster_map of a pointer, and access to what is there, for kernels whose CTAs write to one another's shared memory in bulk
+// (tests/test_peer_rules_cpu.py holds the rules for them).
+__device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank) { return cluster_map(smem_u32(p), rank); }
 __device__ __forceinline__ void peer_store(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
