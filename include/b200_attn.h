@@ -109,8 +109,10 @@ int b200_paged_kv_append_rope(const b200_rope_append_args* args, b200_stream_t s
  * a decode step, a few are the check of a speculated continuation, hundreds a portion of a prompt; a sequence may have none.
  * D 128 or 256, 1 to 64 Q heads per KV head; strides multiples of 8 elements.  cu_seqlens ascends; below zero it names a sequence whose first
  * tokens are in the cache but not among the rows.  Rows outside [cu_seqlens[0], cu_seqlens[batch]) of out are left as they are.  A table
- * entry outside [0, num_pages) reads as zeros.  What the last page holds behind the sequence's end has no influence, not even infinities and
- * NaN.  For a call alone while it runs: workspace, b200_paged_gqa_attention_chunk_workspace_bytes(D) bytes of any content, 16-byte aligned.
+ * entry outside [0, num_pages) reads as zeros; pos below zero counts as zero, and keys for which the table has no room are not seen.  What the
+ * last page holds behind the sequence's end has no influence, not even infinities and NaN; among the values of the new tokens themselves they
+ * may reach the up to 255 new tokens in front as well.  For a call alone while it runs: workspace,
+ * b200_paged_gqa_attention_chunk_workspace_bytes(D) bytes of any content, 16-byte aligned.
  * (The reference prefills from position 0 only: gqa_attention_varlen_causal.py:214.) */
 int64_t b200_paged_gqa_attention_chunk_workspace_bytes(int32_t head_dim);
 typedef struct { /* 8-byte fields only */
@@ -473,9 +475,10 @@ int b200_argmax_rows(const float* logits, int64_t row_stride, int64_t* ids, void
  *   shortest of these prefixes of the order: the first top_k; those with w >= min_p; the fewest whose weights reach top_p of the sum over
  *   what the other two kept.  The first token is always kept.  top_k <= 0 or >= n, min_p <= 0 and top_p >= 1 keep everything.  The id is
  *   the first kept token, by index, at which the running sum of kept weights exceeds uniform times their sum.
- * n up to 524288.  temperature <= 0 or NaN: the largest, ties to the lowest index (as b200_argmax_rows); below 1e-6 it counts as 1e-6, infinity
- * as the largest float.  Several infinities share everything; a row of nothing but -inf and NaN gives 0.  Sums are exact to 2^-31 of a weight, so
- * equal calls give equal ids.  temperature, top_k, top_p, min_p: device arrays [rows], or NULL for the `_all` value.
+ * Up to 65535 rows of n up to 524288.  temperature <= 0 or NaN: the largest, ties to the lowest index (as b200_argmax_rows); below 1e-6 it counts
+ * as 1e-6, infinity as the largest float.  Several infinities share everything; a row of nothing but -inf and NaN gives 0.  Weights are whole
+ * numbers of 2^-44 of the largest, right to about 2^-28 of themselves and one such unit, and added without rounding: equal calls give equal ids.
+ * temperature, top_k, top_p, min_p: device arrays [rows], or NULL for the `_all` value.
  * (The reference only has the arg-max: vocab_argmax.py:141-200.) */
 typedef struct { /* 8-byte fields only */
   const void* logits;

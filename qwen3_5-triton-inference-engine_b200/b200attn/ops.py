@@ -360,7 +360,8 @@ def paged_kv_append_rope(q, k_new, v_new, k_cache, v_cache, block_table, cu_seql
                          freq_axis=None, out=None) -> torch.Tensor:
     """Rotate the new tokens of a packed batch and append their keys and values to the paged cache, one launch -> rotated q.
     q [T, H_q, D], k_new / v_new [T, H_kv, D] bf16, packed by cu_seqlens int32 [B + 1] (a sequence may have no new token); sequence b holds
-    pos[b] tokens (int64 [B], not changed here) and token i of its new ones goes to index pos[b] + i.  position_ids [T] int32 or int64 is
+    pos[b] tokens (int64 [B], not changed here) and token i of its new ones goes to index pos[b] + i.  (cu_seqlens ascends; below zero it names
+    a sequence whose first new tokens are in the cache but not among the rows.)  position_ids [T] int32 or int64 is
     what the rotation sees; or [A, T] with freq_axis int32 [rotary_dim / 2] naming the axis of each frequency (time, height, width; blocks or
     interleaved).  Angles are formed in 64 bits, as positions run far.  D up to 512 and rotary_dim multiples of 16.  Rows outside the
     sequences are left as they are (out too); a token without a page in the table is not written.  out may be q."""
@@ -408,7 +409,8 @@ def paged_gqa_attention_chunk(q, k_cache, v_cache, block_table, cu_seqlens, pos,
     (int64 [B]) before its new ones, whose keys and values are in the cache already (`paged_kv_append_rope`).  One token per sequence is a
     decode step, a few the check of a speculated continuation, hundreds a portion of a prompt, and all of them may share a call.
     gate [T, H_q * D] bf16: the result is multiplied by its sigmoid.  D 128 or 256, up to 64 query heads per key/value head.
-    Rows outside the sequences are left as they are.  What a page holds behind the end of its sequence has no influence."""
+    Rows outside the sequences are left as they are.  What a page holds behind the end of its sequence has no influence; an infinity or NaN
+    among the values of the new tokens may reach the new tokens in front of it."""
     assert q.ndim == 3 and q.dtype == torch.bfloat16
     tokens, num_q_heads, head_dim = q.shape
     assert head_dim == 128 or head_dim == 256, f"head_dim must be 128 or 256, got {head_dim}"
@@ -999,13 +1001,14 @@ def argmax_rows(logits, workspace, out=None, overlap: int = 0) -> torch.Tensor:
 
 
 def sample_rows(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None) -> torch.Tensor:
-    """The next token of every row of logits [rows, n] (fp32 or bf16, n up to 524288), int64 [rows], drawn with uniform fp32 [rows] in [0, 1).
+    """The next token of every row of logits [rows, n] (fp32 or bf16, up to 65535 rows, n up to 524288), int64 [rows], drawn with uniform fp32
+    [rows] in [0, 1).
     Tokens are ordered by logit, larger first, equal ones by index; with w = exp((x - max) / temperature) the shortest of these prefixes is
     kept: the first top_k, those with w >= min_p, the fewest whose weights reach top_p of the sum over what the other two kept.  The id
     is the first kept token, by index, at which the running sum of kept weights exceeds uniform times their sum: equal calls give
     equal ids.  temperature, top_p, min_p (fp32 [rows]) and top_k (int32 [rows]) may differ from row to row, or be plain numbers;
-    top_k <= 0, top_p >= 1 and min_p <= 0 keep everything, temperature <= 0 takes the largest (as `argmax_rows`).  NaN counts as -inf;
-    a row of nothing else gives 0."""
+    top_k <= 0, top_p >= 1 and min_p <= 0 keep everything, temperature <= 0 or NaN takes the largest (as `argmax_rows`), from there to 1e-6 it
+    counts as 1e-6.  NaN among the logits counts as -inf; a row of nothing else gives 0."""
     assert logits.ndim == 2 and logits.dtype in (torch.float32, torch.bfloat16) and logits.shape[1] > 0
     rows, n = logits.shape
     assert n == 1 or logits.stride(1) == 1

@@ -5,7 +5,8 @@
 // Two CTAs of a cluster work on one block of queries after another: the G query heads of a key/value head are stacked into the 128 rows of a
 // CTA's half of an M = 256 tile (row = token * G + head, 128 / G tokens, what is left of the rows idle).  Per 128 keys, cta_group::2:
 //     S[256 x 128]  = Q[256 x D] . K^T           tcgen05.mma, both operands K-major in shared memory, D in TMEM
-//     P = exp2(S * scale * log2e - m)             a thread per row, TMEM -> TMEM (bf16: the operand of the next product; its sum is fp32)
+//     P = exp2(S * scale * log2e - m)             a thread per row, TMEM -> TMEM; bf16, as V is (both operands of a product have one type):
+//                                                 2^-8 of itself at most; its sum is fp32
 //     O[256 x D]   += P[256 x 128] . V[128 x D]   tcgen05.mma, P from TMEM, V as an MN-major operand, O stays in TMEM
 // Each CTA holds 64 keys of a K tile and D/2 columns of a V tile, so a pair fetches a page once.
 //
@@ -13,7 +14,8 @@
 // half pages: a box {64 columns, 8 slots, D/64 blocks} lands as one group of every column block.  Of V a step of 16 keys is a page: a box
 // {64, 16, D/128}.  The page in which a block's keys end is read from a slot below zero, so that its last 16 places hold the last keys and
 // what lies in front is filled with zeros: slots behind the end, which may hold anything, are never read (zeros of P do not help against
-// NaN in V).  Pages that are none, and those behind the end, are boxes outside the pool, zeros too.
+// NaN in V).  Pages that are none, and those behind the end, are boxes outside the pool, zeros too.  (An infinity or NaN among the values of a
+// block's own tokens does make the rows in front of it NaN, whose P is zero there.)
 //
 // Work is cut by keys: all (sequence, kv head, block of queries) rows stand in a line, each as long as its keys and CA_GAP for what a row costs
 // once, and every pair takes an equal stretch.  Lengths are read on the device: nothing the host knows changes from call to call.  A row that a
@@ -24,9 +26,11 @@
 // and PV (even CTA); 13 loads K; 14 walks the line and loads Q and V.  O is rescaled only when a row maximum grows by more than 2^8 (the
 // reference may lag; p then stays below 2^8, which changes no relative rounding).
 //
-// Bound by the exponentials and the tensor pipe in turn (between them a tile's hand-overs), and by the power cap: 8 x 2048 tokens over 2048, 8 + 2
-// heads of 256, 368 to 376 us, 1.10 PFLOP/s of a cuBLAS product's 1.67 (440 in seconds-long runs); 2048 over 30 000 427, 1.22; 16 + 4 heads of 128
-// 370.  Small calls are bound by what lies around: 9 us to the first product, some 4 for the second kernel; 1 x 64 tokens over 500 17 us.
+// Bound by waits of one role for the other at a tile's hand-overs: at 2 x 2048 tokens the tensor pipe works half of the time, the exponential units a
+// quarter; in runs of seconds by the power cap as well.  8 x 2048 tokens over 2048, 8 + 2 heads of 256, 368 to 380 us, 1.09 to 1.12 PFLOP/s of a
+// cuBLAS product's 1.67 (440 in seconds-long runs); 2048 over 30 000 416 to 427, 1.22 to 1.25: the ends of a block's row cost what three tiles do.
+// 16 + 4 heads of 128 371.  Small calls are bound by what lies around: 9 us to the first product, some 4 for the second kernel; 1 x 64 tokens over
+// 500 17 us.
 // (128 keys a tile: two S beside an O of 256 columns fill tensor memory.  Pairs: half the bytes per CTA of K and V through the L2.)
 // Every wait is bounded; on expiry the device error flag is set and the CTA drains.
 #include "chunk.cuh"

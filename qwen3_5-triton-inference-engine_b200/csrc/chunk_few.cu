@@ -4,16 +4,18 @@
 // A block is up to 8 NT query rows of a key/value head (row = token * G + head).  Its pages are the unit of work: one warp, one page,
 // keys as the M dimension of the warp's matrix products, so that few rows cost a narrow N instead of a wide M:
 //     S^T[16 x 8 NT]  = K_page[16 x D] . Q^T[D x 8 NT]              mma.sync m16n8k16, Q^T from shared memory
-//     O^T[D x 8 NT]  += V_page^T[D x 16] . P^T[16 x 8 NT]           P rounded to bf16, its sum in fp32
+//     O^T[D x 8 NT]  += V_page^T[D x 16] . P^T[16 x 8 NT]           P in bf16, as V is (both operands have one type): 2^-8 of itself at
+//                                                                   most; its sum stays in fp32
 // (tcgen05 wants 128 rows, of which 16 would be used; 32 NT small products a page take less than a tenth of the page's time on the bus.)
 // The line of all blocks' pages is cut evenly over one CTA per SM, as in chunk_attention.cu; the eight warps of a CTA take the pages of a
 // piece in turn, each with a K and a V page of its own on their way (128-byte swizzle, one box per page), the next piece's first pages
 // before this one's end.  At a piece's end the warps' states are merged in shared memory.  A block cut between CTAs leaves one partial per
 // CTA, and a second kernel joins them in the order of the keys.  (By the last CTA to arrive, which the first version did, 4 rows over 32 000 keys
 // take 26 us, so 18; 8 rows 40 and 19; nowhere less.)
-// Slots of the last page behind the block's end are cleared in shared memory, for zeros of P do not help against NaN in V.
+// Slots of the last page behind the block's end are cleared in shared memory, for zeros of P do not help against NaN in V.  (An infinity or
+// NaN among the values of a block's own tokens does make the rows in front of it NaN, whose P is zero there.)
 // Every wait is bounded; a CTA that gives up sets the device error flag.
-// Bound by the cache's bytes: 4 x 1 tokens over 30 000 to 32 767, 8 + 2 heads of 256 (251 MB), 47 us, 5.4 TB/s of 6.5; 32 x 4 over 512 to
+// Bound by the cache's bytes: 4 x 1 tokens over 30 000 to 32 767, 8 + 2 heads of 256 (251 MB), 46 us, 5.5 TB/s of 6.5; 32 x 4 over 512 to
 // 4092 (144 MB) 38 us, of which the join is 5.5, launch, lengths, tables and first pages some 6; one token over 10 8.
 #include "chunk.cuh"
 
@@ -362,7 +364,8 @@ chunk_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 }
 
 // Joins the partial sums of cut blocks: grid (slots, CTAs of 64 groups of 4 dimensions of a row), a quarter of the pieces to a thread.
-// (As in chunk_attention.cu, with the units counted first: 1 x 4 tokens over 500 17.0 us, so 15.7; 32 x 4 over 2000 39.6, so 36.)
+// Bound by launch, cuts and one round of loads.  (With the units counted first, as in chunk_attention.cu, 32 x 4 tokens over 2000 took 39.6 us,
+// so 36.)
 constexpr int CJ_QUADS = 64, CJ_SHARES = CF_THREADS / CJ_QUADS;
 template <int DIM>
 __global__ void __launch_bounds__(CF_THREADS)
@@ -408,9 +411,10 @@ chunk_few_join_kernel(const __grid_constant__ ChunkParams p) {
 }
 
 // Calls whose blocks of 16 rows are mostly one per sequence and head, or two where half as many pairs of CTAs are not yet busy with a block each.
-// us here and on pairs: 32 sequences of 16 rows over 2000 keys (2 heads of 256) 36, 53, one over 500 15.7, 15.9; of 32 rows: 32 sequences over
-// 2000 45, 54, 8 over 4000 31, 32, but 64 over 4000 173, 134; 8 of 48 rows over 2000 25.5, 25.4, 16 of them 37, 33.
-// The mean is all that the host knows: 63 single tokens beside a portion of 190 62, 79; but 1000 tokens beside 255 idle sequences 154, 60.
+// us here and on pairs: 32 sequences of 16 rows over 2000 keys (2 heads of 256) 35, 53, one over 500 13.0, 15.0; of 32 rows: 32 sequences over
+// 2000 44, 54, 8 over 4000 29, 32, but 64 over 4000 170, 129; 8 of 48 rows over 2000 24.5, 24.9, 16 of them 36, 33.
+// The mean is all that the host knows: 63 single tokens beside a portion of 190 over 2000 61, 78; but 1000 tokens beside 255 idle sequences
+// over 2000 151, 61, over 30 000 1098, 227, for each block of 16 rows reads the sequence again, where pairs take 256 at a time.
 bool chunk_takes_few(int batch, int tokens, int hkv, int group) {
   const int blocks = static_cast<int64_t>(batch) * hkv * 2 <= sm_count() ? 2 : 1;
   return group <= CF_ROWS && static_cast<int64_t>(tokens) * group <= static_cast<int64_t>(batch) * (CF_ROWS * blocks);

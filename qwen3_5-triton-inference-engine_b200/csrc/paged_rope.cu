@@ -6,8 +6,8 @@
 // Positions run far: the product position * inv_freq in 32 bits is off by half a unit in its last place, 0.004 radians at 100 000, so
 // it is formed in 64 bits, in turns, and only what is left of the last turn goes on in 32 (off by 2^-25 of half a turn).  The pair is
 // rotated in 32 bits and rounded once.
-// Bound: memory; every row is read and written once.  With 10 heads' rows of 256 to rotate and 2 to copy per token 32 768 tokens take 66.5 us,
-// 6.1 TB/s of 6.5, 8300 tokens 20.2 (what a CTA does once, the places and the angles, is a sixth of it), 32 tokens 3.0.  A row in hand and one
+// Bound: memory; every row is read and written once.  With 10 heads' rows of 256 to rotate and 2 to copy per token 32 768 tokens take 67.1 us,
+// 6.0 TB/s of 6.5, 8300 tokens 19.7 (what a CTA does once, the places and the angles, is a sixth of it), 32 tokens 3.1.  A row in hand and one
 // on its way to a thread: four on their way cost 80 registers and 81 us, one at a time with a division per row 69.
 #include "b200_attn.h"
 #include "common.cuh"
